@@ -216,7 +216,7 @@ def _prepare_decode(case, gen, host, s):
         at += size
     pool = need + 3
     ids = host.permutation(pool).astype(np.int32)
-    table = np.zeros((case["batch"], width), np.int32)
+    table = np.full((case["batch"], width), -1, np.int32)
     at, row, first = 0, 0, []
     for size, p in zip(sizes, shared):
         common = ids[at:at + p // page]
@@ -260,7 +260,7 @@ def _prepare_pages(case, gen, host, s):
         lens = _prompt_lengths(case)
         width = -(-(max(lens) + case["tokens"]) // page)
         prompts, rows = case["count"], case["rows"]
-        table = np.zeros((prompts + rows, width), np.int32)
+        table = np.full((prompts + rows, width), -1, np.int32)
         ids = host.permutation(pool).astype(np.int32)
         at = 0
         for i, n in enumerate(lens):
@@ -281,7 +281,7 @@ def _prepare_pages(case, gen, host, s):
         cuts = [live * i // rows for i in range(rows + 1)]
         owned = np.diff(cuts).astype(np.int32)
         width = int(owned.max()) + 2
-        table = np.zeros((rows, width), np.int32)
+        table = np.full((rows, width), -1, np.int32)
         for r in range(rows):
             table[r, :owned[r]] = ids[cuts[r]:cuts[r + 1]]
             # Rows after the first share the page that the first begins with.
@@ -289,7 +289,7 @@ def _prepare_pages(case, gen, host, s):
                 table[r, 1:owned[r] + 1] = table[r, :owned[r]].copy()
                 table[r, 0] = table[0, 0]
                 owned[r] += 1
-        np.add.at(refs, table[np.arange(width)[None] < owned[:, None]], 1)
+        np.add.at(refs, table[table >= 0], 1)
         seq = (owned * page - host.integers(0, page, rows)).astype(np.int32)
     s["table"] = torch.from_numpy(table).cuda()
     s["lens"] = torch.from_numpy(seq).cuda()
@@ -437,11 +437,11 @@ def _plain_fork(s):
     # release
     old = table[dst]
     count(old, cols < owned[dst][:, None], -1)
-    table[dst], lens[dst], owned[dst] = 0, 0, 0
+    table[dst], lens[dst], owned[dst] = -1, 0, 0
     # fork
     used = torch.div(lens[src] + page - 1, page, rounding_mode="floor")
     held = cols < used[:, None]
-    new = torch.where(held, table[src], 0)
+    new = torch.where(held, table[src], -1)
     count(new, held, 1)
     table[dst], lens[dst], owned[dst] = new, lens[src], used.to(owned.dtype)
     # reserve: a shared tail page is copied (its last sharer keeps it when all of them are here), then new pages
@@ -499,7 +499,7 @@ def _plain_compact(s):
     target[torch.where(held, in_order(moves), pool)] = in_order(hole) % pool
     for x in _stored(s):
         x.copy_(x[source[:pool]])
-    new_table = target[table.long()].to(table.dtype)
+    new_table = torch.where(table >= 0, target[table.clamp_min(0).long()].to(table.dtype), table)
     new_refs = torch.where(ids < count, refs[source[:pool]], 0)
     return [new_table, new_refs, count.to(torch.int32).reshape(1)] + _stored(s)
 
