@@ -39,6 +39,8 @@ def device_error(device: torch.device | str | int | None = None) -> int:
     Bit 8 (``FAT_DEVERR_NO_PAGE``): a row asked for more pages than were free, or
     was to append to a page that it does not hold alone.
     Bit 16 (``FAT_DEVERR_BAD_ROW``): a row index outside the page table was skipped.
+    Bit 32 (``FAT_DEVERR_BAD_GROUP``): a ``SharedPrefix`` whose edges fall or leave the
+    batch, or with a group of more than ``max_group`` sequences (decoded without sharing).
     """
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.type == "cuda" and dev.index is None:

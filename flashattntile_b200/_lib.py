@@ -32,6 +32,7 @@ FAT_DEVERR_BAD_PAGE = 2
 FAT_DEVERR_BAD_LENGTH = 4
 FAT_DEVERR_NO_PAGE = 8
 FAT_DEVERR_BAD_ROW = 16
+FAT_DEVERR_BAD_GROUP = 32
 
 DTYPE_CODE = {
     torch.float16: 0,

@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
 
   // Tiles on the line in all, and before the row's group.
   const Line line{p.groups, p.bn, p.num_kv_heads};
-  const bool in_group = p.groups.count > 0 && b < __ldg(p.groups.cu + p.groups.count);
-  const int g = in_group ? p.groups.of(b) : 0;
+  const int found = p.groups.of(b), g = max(found, 0);
+  const bool in_group = found >= 0;
   const int g_first = __shfl_sync(0xffffffffu, g, 0);
   long long all = 0, before = 0;
   for (int i = lane; i < p.groups.count; i += 32) {
@@ -324,7 +324,7 @@ int launch_shared_prefix(const SharedPrefixArgs& a) {
   p.q_bf16 = d.q_dtype == FAT_DTYPE_BF16;
   p.q_negate = d.softmax_scale < 0.f;
   p.scale_log2 = float(std::abs(double(d.softmax_scale)) * 1.4426950408889634);
-  p.groups = Groups{a.cu_groups, a.prefix_lens, a.num_groups, d.batch, d.page_size, cap};
+  p.groups = Groups{a.cu_groups, a.prefix_lens, a.num_groups, d.batch, d.page_size, cap, std::min(a.max_group, d.batch)};
   p.page_table = d.page_table;
   p.pt_sb = d.pt_sb;
   p.max_pages = int(d.max_pages);
@@ -438,7 +438,7 @@ int find_shared_prefix(const int32_t* page_table, int64_t pt_sb, int64_t max_pag
   if (page_table == nullptr || seq_lens == nullptr || cu_groups == nullptr || prefix_out == nullptr)
     return invalid("find_shared_prefix: null pointer argument");
   const int cap = int(std::min<long long>((long long)max_pages * page_size, 1ll << 30));
-  spx::find_kernel<<<num_groups, 256, 0, stream>>>(Groups{cu_groups, nullptr, num_groups, batch, page_size, cap},
+  spx::find_kernel<<<num_groups, 256, 0, stream>>>(Groups{cu_groups, nullptr, num_groups, batch, page_size, cap, batch},
                                                    page_table, pt_sb, cap / page_size, seq_lens, min_sequences,
                                                    prefix_out);
   const cudaError_t e = cudaGetLastError();

@@ -1191,6 +1191,7 @@ __global__ void __launch_bounds__(Layout<Types<TQ, KVT, HD>::D, kMode, Types<TQ,
     const int n = Line{p.groups, L::BN, p.num_kv_heads}.tiles(g);
     tiles += n;
     groups += n > 0;
+    if (blockIdx.x == 0 && !p.groups.sound(g)) raise_error(p.err, FAT_DEVERR_BAD_GROUP);
   }
   for (int b = tid; b < p.groups.batch; b += L::kThreads) {
     int skip;

@@ -23,7 +23,9 @@ The captured step is then: make room for a token (a shared tail page is copied),
 append, shared-prefix decode.  Rows may be released and forked, and the pool
 compacted in place, between replays; where that moves group edges or shortens a
 prefix, write the new values into ``shared.cu_groups`` and ``shared.prefix_lens``
-(a prefix shorter than what is shared is always right).
+(a prefix shorter than what is shared is always right).  No group may grow past the
+``max_group`` that ``shared`` had when the loop was made: a larger one is decoded as if
+it shared nothing, and named in the error word.
 
 Nothing on the host depends on the sequence lengths, so every replay sees the
 lengths the previous one left on the device.  A sequence that reaches the end

@@ -54,7 +54,9 @@ enum {
                                 (max_pages * page_size); it was cut to that capacity   */
   FAT_DEVERR_NO_PAGE = 8,    /* a row asked for more pages than were free, or was to
                                 append to a page that it does not hold alone           */
-  FAT_DEVERR_BAD_ROW = 16    /* a row index outside the page table; it was skipped     */
+  FAT_DEVERR_BAD_ROW = 16,   /* a row index outside the page table; it was skipped     */
+  FAT_DEVERR_BAD_GROUP = 32  /* group edges that fall or leave the batch, or a group of
+                                more than max_group sequences (read without sharing)   */
 };
 
 /* Element types. */
@@ -433,7 +435,10 @@ int fat_compact_pages(const fat_page_pool* pool, int32_t* table_out, int64_t tab
  * tables of a group agree in the first prefix_lens[g] / page_size entries, and none
  * of its sequences is shorter than that many pages (FAT_DEVERR_BAD_LENGTH; the
  * output of a shorter one is then not meaningful).  A prefix that ends inside a page
- * is used up to the page's start.  max_group bounds the groups' sizes.
+ * is used up to the page's start.  No group has more than max_group sequences; one
+ * that does is decoded as if it shared nothing (FAT_DEVERR_BAD_GROUP).  Where edges
+ * fall (FAT_DEVERR_BAD_GROUP too) the output of the sequences that two groups claim is
+ * not meaningful.
  *
  * `decode` holds the arguments of fat_paged_decode_call (lse and the stats_* fields
  * are not used; workspace as there).  scratch: fat_shared_prefix_scratch_size bytes

@@ -1,0 +1,63 @@
+"""Shared-prefix decode where its inputs are at the edge of what they may be.
+
+Bounds as in ``test_shared_prefix_gpu`` (one softmax per sequence and head in 64 bits).
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_shared_prefix_gpu import DEV, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import flashattntile_b200  # noqa: F401
+
+
+def _edges(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("kind", ["f16", "int8"])
+@pytest.mark.parametrize("most", [0, 1, 15, 16, 39])
+def test_a_group_larger_than_announced(kind, most):
+    """It is decoded without sharing, and named; the groups beside it share."""
+    from flashattntile_b200 import SharedPrefix, device_error, shared_prefix_decode_attention, value_checks
+
+    q, cache, scales = make(kind, [40, 2], [320, 96], [1 + i % 7 for i in range(42)], 32, 4, 128, 16, seed=most)
+    shared = SharedPrefix(_edges(0, 40, 42), _edges(320, 96), most)
+    with value_checks(False):
+        out = shared_prefix_decode_attention(q, cache, shared, scales=scales)
+        assert device_error() == 32
+        check(out, q, cache, scales)
+
+
+def test_edges_that_do_not_start_at_the_first_sequence():
+    """Sequences before the first edge are in no group."""
+    from flashattntile_b200 import SharedPrefix, shared_prefix_decode_attention, value_checks
+
+    q, cache, _ = make("f16", [40], [320], [1 + i % 7 for i in range(40)], 32, 4, 128, 16, seed=1)
+    for first in (1, 39):
+        with value_checks(False):
+            out = shared_prefix_decode_attention(q, cache, SharedPrefix(_edges(first, 40), _edges(320), 40))
+        check(out, q, cache, None)
+
+
+def test_edges_that_fall_or_leave_the_batch_are_named():
+    from flashattntile_b200 import SharedPrefix, device_error, shared_prefix_decode_attention, value_checks
+
+    q, cache, _ = make("f16", [6], [64], [1, 2, 3, 4, 5, 6], 8, 2, 64, 16, seed=1)
+    want = shared_prefix_decode_attention(q, cache, SharedPrefix(_edges(0, 6), _edges(64), 6))
+    for edges in ((0, 4, 2), (0, 4, 9), (-3, 3, 6), (5, 0, 6), (7, 7, 7)):
+        with value_checks(False):
+            out = shared_prefix_decode_attention(q, cache, SharedPrefix(_edges(*edges), _edges(64, 64), 6))
+            assert device_error() == 32
+            assert out.shape == want.shape and out.isfinite().all()
+    # A call after them is right.
+    assert torch.equal(shared_prefix_decode_attention(q, cache, SharedPrefix(_edges(0, 6), _edges(64), 6)), want)
