@@ -69,6 +69,10 @@ constexpr float kRescaleLog2 = 8.f;    // running-max slack before O is rescaled
 // P is held in units of 2^-7, so at most 2^15: what is small beside a heavy key stays
 // normal in fp16 for as long as it can.
 constexpr float kLiftLog2 = 7.f;
+// 8-bit: a V scale below the normal floats, or below 2^-100 of a larger one before it or in
+// its tile, counts as 0 (P in units of the larger one would leave fp32).
+constexpr float kLeastScale = 1.17549435e-38f;
+constexpr float kLeastRatio = 7.8886091e-31f;
 constexpr long long kMaxTiles = (1ll << 31) - 1;  // tiles on the line (2^38 tokens times KV heads)
 
 // Streams: two row tiles, one row tile with half of each tile's tokens each, or one
@@ -136,8 +140,8 @@ struct Layout {
       (kMode == kRowPair ? (k8 ? 2.6f : 3.3f) : (k8 ? 1.4f : 1.7f)) * (D == 64 ? 0.75f : 1.f);
   static constexpr int kBars = 4 + 2 * kStagesK + 2 * kStagesV + 6 * kStreams + 3 + 2 * kStagesRaw +
                                (k8 ? kScaleSlots : 0);
-  // Per 8 tokens: K scale, log2 of the V scale's size, its reciprocal; then the
-  // largest V scale and the K and V masks (bits 0-15 zero, 16-31 negative).
+  // Per 8 tokens: K scale, log2 of the V scale's size in units, its reciprocal; then the
+  // unit and the K and V masks (bits 0-15 zero, 16-31 negative).
   static constexpr int kScaleRow = 3 * (BN / 8) + 4;
   static constexpr int kScaleFloats = k8 ? kScaleSlots * kScaleRow : 0;
   static constexpr size_t kData = size_t(kRowTiles) * kQTile + size_t(kStagesK + kStagesV) * kTile +
@@ -511,6 +515,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
         page1 = checked(page1, slot1);
         float ks1, vs1;
         scales_of(page1, ks1, vs1);
+        [[maybe_unused]] float unit = 0.f;  // 8-bit: what O is in units of (the piece's V scales so far)
         for (int j = w.t0; j < w.t1; ++j) {
           const int page = page1, slot0 = slot1;
           [[maybe_unused]] const float ks = ks1, vs = vs1;
@@ -555,9 +560,11 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
             }
           } else {
             // Raw K, then raw V; beside them, per 8 tokens: the K scale, and for the V
-            // scale f its logarithm (P f = 2^(x + log2 f): no product per element) and
-            // 1 / f (which takes f out of the sum of P again), and the tile's largest f.
-            // Where no page is, or where a scale is 0, the tile's codes count as zeros.
+            // scale f in units of `unit`, a power of two above every f of the piece so far,
+            // log2(f / unit) (P f / unit = 2^(x + log2(f / unit)): no product per element)
+            // and unit / f (which takes f out of the sum of P again); then the unit.
+            // Where no page is, or where a scale is 0, the tile's codes count as zeros; P of
+            // a zero V scale is in the unit itself, so that it is as finite as the others'.
             const int slot = issued % L::kScaleSlots;
             const int per8 = p.box_rows / 8;
 #pragma unroll
@@ -570,13 +577,14 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
                 // The slot's previous tile left the softmax before its raw stage came free.
                 const float kg = __shfl_sync(0xffffffffu, ks, (lane / per8) & 31);
                 const float vg = __shfl_sync(0xffffffffu, vs, (lane / per8) & 31);
-                float vm = lane < kGroups8 ? fabsf(vg) : 0.f;
+                const float f = fabsf(vg);
+                float vm = lane < kGroups8 && f >= kLeastScale && f < CUDART_INF_F ? f : 0.f;
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+                vm = __shfl_sync(0xffffffffu, vm, 0);
+                if (vm > unit) unit = __int_as_float(min(254, ((__float_as_int(vm) >> 23) & 0xFF) + 1) << 23);
                 float* sc = scales + slot * L::kScaleRow;
-                // A V scale below the normal floats counts as 0.
-                const float f = fabsf(vg);
-                const bool none = f < 1.17549435e-38f;
+                const bool none = f < fmaxf(kLeastScale, unit * kLeastRatio);
                 const unsigned in = (1u << kGroups8) - 1u;
                 const unsigned kmask = (__ballot_sync(0xffffffffu, kg == 0.f) & in) |
                                        ((__ballot_sync(0xffffffffu, kg < 0.f) & in) << 16);
@@ -584,11 +592,11 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
                                        ((__ballot_sync(0xffffffffu, vg < 0.f) & in) << 16);
                 if (lane < kGroups8) {
                   sc[lane] = fabsf(kg);
-                  sc[kGroups8 + lane] = none ? 0.f : log2f(f);
-                  sc[2 * kGroups8 + lane] = none ? 1.f : 1.f / f;
+                  sc[kGroups8 + lane] = none ? 0.f : log2f(f) - float((__float_as_int(unit) >> 23) - 127);
+                  sc[2 * kGroups8 + lane] = none ? 1.f : unit / f;
                 }
                 if (lane == 0) {
-                  sc[3 * kGroups8] = vm;
+                  sc[3 * kGroups8] = unit;
                   sc[3 * kGroups8 + 1] = __uint_as_float(kmask);
                   sc[3 * kGroups8 + 2] = __uint_as_float(vmask);
                 }
@@ -915,8 +923,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
       const bool active = kMode != kRowPair || t * p.tile_rows < w.rows;
       const int left = w.tokens - w.t0 * BN;  // shared tokens from the piece's first tile on
       float m_used = -CUDART_INF_F, l_sum = 0.f;
-      float vref = 0.f;  // 8-bit: O is in units of this power of two (at least every V scale seen)
-      [[maybe_unused]] float vlog = 0.f;  // its logarithm
+      float vref = 0.f;  // 8-bit: O is in units of this power of two (0: of any, it is all zeros)
       const int U = active ? n * L::kUnits : 0;
       for (int u = 0; u < U; ++u, ++x) {
         const int b = x & 1;
@@ -1004,7 +1011,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
         } else {
           // The K scale of an 8-token group multiplies its scores; its V scale f, in
           // units of vref, multiplies P as 2^(x + log2(f / vref)) and leaves the sum of P
-          // by vref / f.
+          // by vref / f (both from the producer).
           const int slot = (tile + j) % L::kScaleSlots;
           if (!wait(sc_full + 8 * slot, ((tile + j) / L::kScaleSlots) & 1)) {
             ok = false;
@@ -1034,21 +1041,17 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
             }
           }
           raise_max(mx * kq);
-          // O's unit grows to a power of two above the largest V scale so far.
-          const float vm = scales[slot * L::kScaleRow + 3 * kGroups8];
-          if (vm > vref && vm < CUDART_INF_F) {
-            const int e = min(254, ((__float_as_int(vm) >> 23) & 0xFF) + 1);
-            const float up = __int_as_float(e << 23);
+          // O's unit only grows.
+          const float unit = scales[slot * L::kScaleRow + 3 * kGroups8];
+          if (unit > vref) {
             if (vref > 0.f) {
-              factor *= vref / up;
+              factor *= vref / unit;
               grow = true;
             }
-            vref = up;
-            vlog = float(e - 127);
+            vref = unit;
           }
           if (!(ok = rescale())) break;
-          const float msub = ((m_used == -CUDART_INF_F) ? 0.f : m_used - kLiftLog2) + vlog;
-          const float unit = vref > 0.f ? vref : 1.f;
+          const float msub = (m_used == -CUDART_INF_F) ? 0.f : m_used - kLiftLog2;
 #pragma unroll
           for (int q4 = 0; q4 < 2; ++q4) {
             const float4 k4 = sc[2 * half + q4], l4 = sc[kQuads + 2 * half + q4], i4 = sc[2 * kQuads + 2 * half + q4];
@@ -1067,9 +1070,8 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
                 fma2(x0, x1, __uint_as_float(y[i]), __uint_as_float(y[i + 1]), kf, sub);
                 packed[(q4 * 4 + g8) * 4 + i / 2] = pack_p(fast_exp2(x0), fast_exp2(x1), e0, e1);
               }
-              const float w8 = ig[g8] * unit;
-              sum0 = fmaf(e0, w8, sum0);
-              sum1 = fmaf(e1, w8, sum1);
+              sum0 = fmaf(e0, ig[g8], sum0);
+              sum1 = fmaf(e1, ig[g8], sum1);
             }
           }
           tc::st32(lane_base + colS, packed);
