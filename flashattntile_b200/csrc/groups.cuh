@@ -28,26 +28,29 @@ struct Groups {
     return a >= 0 && b >= a && b <= batch && b - a <= max_size;
   }
 
-  // The group of sequence b, or -1.  The search takes the last group that starts at or
-  // before b (empty groups start where the next one does); whatever the edges hold, the
-  // group that it returns has b inside, so that a row's place in its group is one that
-  // the launch has room for.
-  __device__ __forceinline__ int of(int b) const {
-    if (count <= 0 || b >= __ldg(cu + count)) return -1;
+  // The last group that starts at or before b (empty groups start where the next one does).
+  __device__ __forceinline__ int near(int b) const {
     int lo = 0, hi = count - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (__ldg(cu + mid) <= b) lo = mid;
       else hi = mid - 1;
     }
-    const int a = first(lo), e = first(lo + 1);
-    return b >= a && b < e && e - a <= max_size ? lo : -1;
+    return lo;
   }
 
-  // Shared tokens of sequence b (0 without a group).
+  // Whether group g, whatever the edges hold, has b inside and no more sequences than the
+  // launch has room for, so that b's rows have a place in it.
+  __device__ __forceinline__ bool has(int g, int b) const {
+    const int a = first(g), e = first(g + 1);
+    return b >= a && b < e && e - a <= max_size;
+  }
+
+  // Shared tokens of sequence b (0 without a group).  Its loads are independent after the search.
   __device__ __forceinline__ int tokens_of(int b) const {
-    const int g = of(b);
-    return g < 0 ? 0 : tokens(g);
+    if (count <= 0) return 0;
+    const int g = near(b), t = tokens(g);
+    return has(g, b) ? t : 0;
   }
 };
 

@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
 
   // Tiles on the line in all, and before the row's group.
   const Line line{p.groups, p.bn, p.num_kv_heads};
-  const int found = p.groups.of(b), g = max(found, 0);
-  const bool in_group = found >= 0;
+  const int g = p.groups.count > 0 ? p.groups.near(b) : 0;
+  const bool in_group = p.groups.count > 0 && p.groups.has(g, b);
   const int g_first = __shfl_sync(0xffffffffu, g, 0);
   long long all = 0, before = 0;
   for (int i = lane; i < p.groups.count; i += 32) {
