@@ -37,8 +37,7 @@
 //   8 sequences of 133k tokens, 131k shared, 64/8 heads of 128, fp16: 568 MB in 115 us,
 //     4.9 TB/s.  The prefix phase runs at memory speed; 5 us of start, 9 us of join.
 //   64 sequences of 8k + up to 1k tokens, 32/8 heads, bf16: 196 MB in 59 us.  The own
-//     tokens are two thirds of the bytes: latency of single warps.  (P of bf16 as two
-//     parts costs nothing there once the shares of the CTAs allow for it.)
+//     tokens are two thirds of the bytes: latency of single warps.
 //   128 sequences of 16k + up to 512, 32/8 heads, int8: 101 MB in 101 us: a 16k prefix
 //     against 512 rows is compute, and the softmax of 8-bit tiles (scales per 8 tokens)
 //     takes 1.4 us per unit of both streams, where a 16-bit one takes 0.85.
@@ -135,9 +134,10 @@ struct Layout {
   static_assert(!kSplitRegs || !k8 || 384 * kRegsOwn + (kThreads - 384) * kRegsIdle <= kThreads * kLaunchRegs,
                 "register split exceeds the launch");
   // What a tile costs a CTA, in units of 32 KB of own tokens.  Swept over sixteen shapes:
-  // these are within 6% of each one's best, half or twice them costs up to 50%.
+  // half or twice them costs up to 50%; over 28 more (head_dim 64 and 128), 0.87 to 1.2
+  // times them measures within 3%.
   static constexpr float kTileCost =
-      (kMode == kRowPair ? (k8 ? 2.6f : 3.3f) : (k8 ? 1.4f : 1.7f)) * (D == 64 ? 0.75f : 1.f);
+      (kMode == kRowPair ? (k8 ? 3.0f : 3.8f) : (k8 ? 1.4f : 1.95f)) * (D == 64 ? 0.75f : 1.f);
   static constexpr int kBars = 4 + 2 * kStagesK + 2 * kStagesV + 6 * kStreams + 3 + 2 * kStagesRaw +
                                (k8 ? kScaleSlots : 0);
   // Per 8 tokens: K scale, log2 of the V scale's size in units, its reciprocal; then the
@@ -242,31 +242,25 @@ struct Walk {
   }
 };
 
-// s0 += low half of h, s1 += high half.
-__device__ __forceinline__ void add_half2(float& s0, float& s1, uint32_t h) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.f16 %0, a, %0;\n\tadd.rn.f32.f16 %1, b, %1;\n\t}"
-      : "+f"(s0), "+f"(s1)
-      : "r"(h));
-}
-
-// P's fp16 pair and the sum of what enters P.V.  The sum is taken over the bits that
-// P.V sees, so that the weights sum to one exactly: a row with one heavy key loses
-// nothing (sums of unrounded P cost such a row up to 2^-11).  Rounded, not cut: what is
-// small beside a heavy key is subnormal, where cutting would lean to one side.
-__device__ __forceinline__ uint32_t pack_p(float p0, float p1, float& s0, float& s1) {
-  const uint32_t h = pack2<__half>(p0, p1);
-  add_half2(s0, s1, h);
-  return h;
-}
-
-// bf16 keeps 8 bits of a probability, which cost a result up to as much again as its own
-// rounding to bf16 does.  So P enters as two parts, the cut value and the remainder
-// (2^-17 is left out), in two products: the tensor core has the time.
+// Two probabilities for P.V, as two 16-bit parts in two products: what the type keeps of
+// them (cut: bf16 8 bits, fp16 11) and the remainder, of which 2^-17 or 2^-21 of the whole
+// is left out; s0 and s1 sum them in 32 bits.  One part alone costs a result up to as much
+// again as its own rounding to the type, and in 8-bit caches, where P carries the V scale,
+// a group whose scale is far below its neighbours' would vanish from a sum of rounded P.
+// The tensor core has the time.
+template <typename T>
 __device__ __forceinline__ uint32_t split_p(float p0, float p1, float& s0, float& s1, uint32_t& rest) {
-  const uint32_t a = __float_as_uint(p0) & 0xffff0000u, b = __float_as_uint(p1) & 0xffff0000u;
+  constexpr uint32_t kKeep = std::is_same<T, __nv_bfloat16>::value ? 0xffff0000u : 0xffffe000u;
+  float r0 = p0, r1 = p1;  // less the cut values: probabilities have no sign, so one operation each
+  add2(r0, r1, __uint_as_float((__float_as_uint(p0) & kKeep) | 0x80000000u),
+       __uint_as_float((__float_as_uint(p1) & kKeep) | 0x80000000u));
   add2(s0, s1, p0, p1);
-  rest = pack2<__nv_bfloat16>(p0 - __uint_as_float(a), p1 - __uint_as_float(b));
-  return __byte_perm(a, b, 0x7632);
+  rest = pack2<T>(r0, r1);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+  uint32_t h;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(p1), "f"(p0));
+  return h;
 }
 
 // True in one thread of a whole warp, in a form that the compiler knows to be one thread.
@@ -328,7 +322,6 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
   constexpr int BN = L::BN, SK = L::kStagesK, SV = L::kStagesV, SR = L::kStagesRaw;
   constexpr int NS = L::kStreams;
   constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-  constexpr bool kSplitP = fmt == 1;  // bf16: P as two parts
   constexpr uint32_t kIdescQK = tc::idesc_f16(BM, kUnit, fmt, 0, 0);
   constexpr uint32_t kIdescPV = tc::idesc_f16(BM, D, fmt, 0, 1);
   constexpr int kGroups8 = BN / 8;  // 8-token groups of a tile (a page holds whole ones)
@@ -674,7 +667,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
       auto issue_pv = [&](int t, int b, uint32_t loV, int h, bool acc) {
         loV += uint32_t(h) * (uint32_t(kUnit * 128) >> 4);
 #pragma unroll
-        for (int kk = 0; kk < (kSplitP ? 2 : 1) * kUnit / 16; ++kk) {
+        for (int kk = 0; kk < 2 * kUnit / 16; ++kk) {
           const int tok = kk % (kUnit / 16) * 16;  // the remainders of P follow the cut values
           tc::mma_ts(tmem + kColO + 128 * t, tmem + 128 * t + kUnit * b + kk * 8,
                      desc(loV + uint32_t((tok * 128) >> 4), hiV), kIdescPV, (acc || kk > 0) ? 1u : 0u);
@@ -991,23 +984,17 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
           }
           if (!(ok = rescale())) break;
           const float msub = (m_used == -CUDART_INF_F) ? 0.f : m_used - kLiftLog2;
-          uint32_t packed[32];
-          [[maybe_unused]] uint32_t rest[kSplitP ? 32 : 1];
+          uint32_t packed[32], rest[32];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float x0, x1, x2, x3;
             fma2(x0, x1, s[2 * i], s[2 * i + 1], p.scale_log2, -msub);
             fma2(x2, x3, s[2 * i + 2], s[2 * i + 3], p.scale_log2, -msub);
-            if constexpr (kSplitP) {
-              packed[i] = split_p(fast_exp2(x0), fast_exp2(x1), sum0, sum1, rest[i]);
-              packed[i + 1] = split_p(fast_exp2(x2), fast_exp2(x3), sum2, sum3, rest[i + 1]);
-            } else {
-              packed[i] = pack_p(fast_exp2(x0), fast_exp2(x1), sum0, sum1);
-              packed[i + 1] = pack_p(fast_exp2(x2), fast_exp2(x3), sum2, sum3);
-            }
+            packed[i] = split_p<T>(fast_exp2(x0), fast_exp2(x1), sum0, sum1, rest[i]);
+            packed[i + 1] = split_p<T>(fast_exp2(x2), fast_exp2(x3), sum2, sum3, rest[i + 1]);
           }
           tc::st32(lane_base + colS, packed);
-          if constexpr (kSplitP) tc::st32(lane_base + colS + 32, rest);
+          tc::st32(lane_base + colS + 32, rest);
         } else {
           // The K scale of an 8-token group multiplies its scores; its V scale f, in
           // units of vref, multiplies P as 2^(x + log2(f / vref)) and leaves the sum of P
@@ -1022,7 +1009,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
           constexpr int kQuads = kGroups8 / 4;
           const float kq = p.scale_log2 * qmul;
           float mx = -CUDART_INF_F;
-          uint32_t r[2][32], packed[32];
+          uint32_t r[2][32], packed[32], rest[32];
           tc::ld32(lane_base + colS, r[0]);
           tc::ld32(lane_base + colS + 32, r[1]);
           tc::wait_ld();
@@ -1068,13 +1055,15 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
               for (int i = 0; i < 8; i += 2) {
                 float x0, x1;
                 fma2(x0, x1, __uint_as_float(y[i]), __uint_as_float(y[i + 1]), kf, sub);
-                packed[(q4 * 4 + g8) * 4 + i / 2] = pack_p(fast_exp2(x0), fast_exp2(x1), e0, e1);
+                const int at = (q4 * 4 + g8) * 4 + i / 2;
+                packed[at] = split_p<T>(fast_exp2(x0), fast_exp2(x1), e0, e1, rest[at]);
               }
               sum0 = fmaf(e0, ig[g8], sum0);
               sum1 = fmaf(e1, ig[g8], sum1);
             }
           }
           tc::st32(lane_base + colS, packed);
+          tc::st32(lane_base + colS + 32, rest);
         }
         l_sum += (sum0 + sum1) + (sum2 + sum3);
         tc::wait_st();
@@ -1227,8 +1216,7 @@ __global__ void __launch_bounds__(Layout<Types<TQ, KVT, HD>::D, kMode, Types<TQ,
     tiles = 0;
   }
   const int units = p.num_kv_heads * d.head_groups;
-  constexpr float kCost = L::kTileCost * (std::is_same<typename Y::T, __nv_bfloat16>::value ? 1.15f : 1.f);  // split P
-  const float work_p = float(tiles) * p.per_gang * kCost;
+  const float work_p = float(tiles) * p.per_gang * L::kTileCost;
   const float work_o = float(tokens) * units * (2.f * LO::kRowBytes / 32768.f);
   const int gangs = choose_gangs(tiles, groups == 1 ? p.num_kv_heads : 0, int(gridDim.x), p.per_gang, work_p, work_o);
   const int piece = own::piece_tokens(tokens, units, d.workers, LO::kTokens);

@@ -80,3 +80,19 @@ def test_scales_of_either_sign_and_k_scales_of_zero(kind, shape):
         y = x.float().clamp(-127 if kind == "int8" else -448, 448) * sign[n][:, None, :, None]
         x.copy_(y.to(x.dtype))
     check(out, q, cache, scales)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("small,codes", [(1e-8, False), (1e-8, True), (2.0 ** -18, True), (2.0 ** -120, True)])
+def test_v_scales_far_apart(kind, shape, small, codes):
+    """Half of the pages hold values that are zero (``codes`` false) or next to nothing; 1e-8
+    is the least scale that quantisation gives.  Their weights stay in the sum."""
+    for seed in range(3):
+        sizes, q, cache, scales = _case(kind, shape, seed=seed, spread=2.0)
+        gen = torch.Generator(device=DEV).manual_seed(seed + 50)
+        pages = torch.rand(cache.num_pages, generator=gen, device=DEV) < 0.5
+        scales["v"][pages] = small
+        if not codes:
+            cache.v_cache.view(torch.uint8)[pages] = 0
+        check(_decode(q, cache, scales, sizes), q, cache, scales)
