@@ -134,10 +134,12 @@ struct Layout {
   static_assert(!kSplitRegs || !k8 || 384 * kRegsOwn + (kThreads - 384) * kRegsIdle <= kThreads * kLaunchRegs,
                 "register split exceeds the launch");
   // What a tile costs a CTA, in units of 32 KB of own tokens.  Swept over sixteen shapes:
-  // half or twice them costs up to 50%; over 28 more (head_dim 64 and 128), 0.87 to 1.2
-  // times them measures within 3%.
+  // half or twice them costs up to 50%; over 28 more (head_dim 64 and 128), up to 1.35
+  // times them measures within 3%.  8-bit pairs sit beside a step: 512 rows, 16k shared and
+  // up to 512 own tokens take 106 us, 115 with 3.0, where prefix CTAs come to the own tokens
+  // when a few are left.
   static constexpr float kTileCost =
-      (kMode == kRowPair ? (k8 ? 3.0f : 3.8f) : (k8 ? 1.4f : 1.95f)) * (D == 64 ? 0.75f : 1.f);
+      (kMode == kRowPair ? (k8 ? 2.6f : 3.8f) : (k8 ? 1.4f : 1.95f)) * (D == 64 ? 0.75f : 1.f);
   static constexpr int kBars = 4 + 2 * kStagesK + 2 * kStagesV + 6 * kStreams + 3 + 2 * kStagesRaw +
                                (k8 ? kScaleSlots : 0);
   // Per 8 tokens: K scale, log2 of the V scale's size in units, its reciprocal; then the

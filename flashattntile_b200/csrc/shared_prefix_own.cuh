@@ -32,6 +32,7 @@ namespace own {
 
 constexpr int kRows = 8;             // query heads per piece
 constexpr float kRescaleLog2 = 8.f;  // running-max slack before O is rescaled
+constexpr float kLift = 64.f;        // 8-bit: P is held in units of 1 / kLift
 constexpr int kPiecesPerWarp = 4;    // pieces for each of 8 warps per CTA at most (and one per unit)
 
 template <int KVT>
@@ -277,6 +278,9 @@ __device__ __forceinline__ void own_body(const CUtensorMap& tm_k, const CUtensor
   float o[NT][4];                          // columns d of rows g, g + 8 of the tile; heads 2c, 2c + 1
   float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;  // of heads 2c, 2c + 1
   float qmul0 = 1.f, qmul1 = 1.f;
+  // 8-bit: P carries the V scale in units of a power of two above every one of the piece so
+  // far, times kLift, so that it neither leaves fp16 nor loses bits, whatever V's size.
+  float vunit = 0.f, vinv = 0.f;
   uint32_t qb[D / 16][2];
   int done = 0;
   while (done < issued) {
@@ -291,6 +295,7 @@ __device__ __forceinline__ void own_body(const CUtensorMap& tm_k, const CUtensor
     if (flags & 1) {
       m0 = m1 = -CUDART_INF_F;
       l0 = l1 = 0.f;
+      vunit = vinv = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
       const int b = note[1], unit = note[2];
@@ -449,6 +454,27 @@ __device__ __forceinline__ void own_body(const CUtensorMap& tm_k, const CUtensor
         mx0 = fmaxf(mx0, s0[r]);
         mx1 = fmaxf(mx1, s1[r]);
       }
+      if constexpr (EB == 1) {
+        float vm = 0.f;  // the same in every lane
+#pragma unroll
+        for (int r = 0; r < 2 * kSteps; ++r) {
+          const float f = fabsf(vf[r]);
+          vm = fmaxf(vm, f >= 1.17549435e-38f && f < CUDART_INF_F ? f : 0.f);
+        }
+        if (vm > vunit) {
+          const int e = min(253, ((__float_as_int(vm) >> 23) & 0xFF) + 1);
+          const float up = __int_as_float(e << 23), a = vunit / up;  // o is 0 before the first unit
+          vunit = up;
+          vinv = __int_as_float((254 - e) << 23) * kLift;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= a;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2 * kSteps; ++r) vf[r] *= vinv;
+      }
       if (__any_sync(0xffffffffu, mx0 > m0 + kRescaleLog2 || mx1 > m1 + kRescaleLog2)) {
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) {
@@ -538,6 +564,10 @@ __device__ __forceinline__ void own_body(const CUtensorMap& tm_k, const CUtensor
       float* at = p.part_o + (x * (D / 4) * p.rows + h0) * 4;
       auto put = [&](int d, float y0, float y1) {
         float* to = at + (long long)(d >> 2) * p.rows * 4 + (d & 3);
+        if constexpr (EB == 1) {
+          y0 *= vunit * (1.f / kLift);
+          y1 *= vunit * (1.f / kLift);
+        }
         if (h0 < rows) to[0] = y0;
         if (h0 + 1 < rows) to[4] = y1;
       };

@@ -67,6 +67,10 @@ SHAPES = [  # sizes, prefixes, own tokens, heads, kv heads, dim, page
     ([40], [1040], [1 + i % 9 for i in range(40)], 16, 2, 64, 8),    # two row tiles
     ([3, 2], [768, 512], [10, 30, 0, 1, 57], 4, 2, 256, 32),         # one stream
     ([6], [640], [1, 2, 3, 4, 5, 6], 8, 4, 32, 16),
+    ([4, 2], [400, 96], [3, 40, 17, 90, 2, 70], 24, 2, 128, 8),      # 12 heads per KV head: two head groups
+    ([2], [256], [100, 30], 64, 1, 64, 16),                          # 64: eight
+    ([2, 1], [96, 0], [9, 300, 80], 128, 1, 64, 32),                 # 128: one sequence per row tile
+    ([5], [336], [1, 20, 3, 40, 5], 27, 3, 64, 16),                  # 9: a head group of one
 ]
 
 
@@ -86,3 +90,24 @@ def test_weights_are_kept(kind, shape):
         over = (out.double() - want).abs() / (bound + 2.0 ** -40)
         assert float(over.max()) <= 1.0, f"{float(over.max()):.2f} of its bound"
         assert device_error() == 0
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("size", [-30, -12, 12, 30])
+def test_values_of_any_size(kind, dim, size):
+    """V scales of 2^-40 to 2^30, in the prefix and in own tokens, rising and falling along them."""
+    from flashattntile_b200 import device_error, find_shared_prefix, shared_prefix_decode_attention
+
+    q, cache, scales = make(kind, [3], [320], [0, 40, 300], 8, 2, dim, 16, seed=dim, spread=2.0)
+    scales["v"] *= 2.0 ** size
+    for own in (1, 2):  # larger page by page, then smaller
+        n = -(-int(cache.seq_lens[own]) // 16)
+        steps = torch.arange(n, device=DEV, dtype=torch.float32)
+        scales["v"][cache.page_table[own, :n].long()] *= torch.exp2(steps % 11 - 5 if own == 1 else 5 - steps % 11)[:, None]
+    out = torch.empty(q.shape, dtype=torch.float32, device=DEV)
+    shared_prefix_decode_attention(q, cache, find_shared_prefix(cache, [3]), scales=scales, out=out)
+    want, bound = _exact(q, cache, scales)
+    assert out.isfinite().all()
+    assert float(((out.double() - want).abs() / (bound + 2.0 ** (size - 40))).max()) <= 1.0
+    assert device_error() == 0
