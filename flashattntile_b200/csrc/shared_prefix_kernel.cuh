@@ -969,9 +969,12 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
 #pragma unroll
             for (int i = 0; i < kUnit; ++i) s[i] = __uint_as_float(r[i / 32][i % 32]);
           }
+          float mul = p.scale_log2;
           if (lim < kUnit) {
+            // Masked after the product: the scale may be 0.
+            mul = 1.f;
 #pragma unroll
-            for (int i = 0; i < kUnit; ++i) s[i] = i < lim ? s[i] : -CUDART_INF_F;
+            for (int i = 0; i < kUnit; ++i) s[i] = i < lim ? s[i] * p.scale_log2 : -CUDART_INF_F;
           }
           {
             float a0 = fmaxf(s[0], s[4]), a1 = fmaxf(s[1], s[5]), a2 = fmaxf(s[2], s[6]), a3 = fmaxf(s[3], s[7]);
@@ -982,7 +985,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
               a2 = max3(a2, s[i + 2], s[i + 6]);
               a3 = max3(a3, s[i + 3], s[i + 7]);
             }
-            raise_max(fmaxf(max3(a0, a1, a2), a3) * p.scale_log2);
+            raise_max(fmaxf(max3(a0, a1, a2), a3) * mul);
           }
           if (!(ok = rescale())) break;
           const float msub = (m_used == -CUDART_INF_F) ? 0.f : m_used - kLiftLog2;
@@ -990,8 +993,8 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float x0, x1, x2, x3;
-            fma2(x0, x1, s[2 * i], s[2 * i + 1], p.scale_log2, -msub);
-            fma2(x2, x3, s[2 * i + 2], s[2 * i + 3], p.scale_log2, -msub);
+            fma2(x0, x1, s[2 * i], s[2 * i + 1], mul, -msub);
+            fma2(x2, x3, s[2 * i + 2], s[2 * i + 3], mul, -msub);
             packed[i] = split_p<T>(fast_exp2(x0), fast_exp2(x1), sum0, sum1, rest[i]);
             packed[i + 1] = split_p<T>(fast_exp2(x2), fast_exp2(x3), sum2, sum3, rest[i + 1]);
           }

@@ -61,3 +61,17 @@ def test_edges_that_fall_or_leave_the_batch_are_named():
             assert out.shape == want.shape and out.isfinite().all()
     # A call after them is right.
     assert torch.equal(shared_prefix_decode_attention(q, cache, SharedPrefix(_edges(0, 6), _edges(64), 6)), want)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("rows,dim", [(3, 128), (40, 64), (3, 256), (5, 32)])  # one row tile, two, one stream
+def test_any_scale_on_a_prefix_that_ends_inside_a_tile(kind, rows, dim):
+    """Masked scores stay masked, also by a scale of 0 (then every token weighs the same)."""
+    from flashattntile_b200 import find_shared_prefix, shared_prefix_decode_attention
+
+    for tokens in (16, 80, 128, 656):
+        q, cache, scales = make(kind, [rows], [tokens], [1 + i % 3 for i in range(rows)], 16, 4, dim, 16, seed=tokens)
+        shared = find_shared_prefix(cache, [rows])
+        for scale in (0.0, -0.0, 0.02, -0.3, 1e-38):
+            check(shared_prefix_decode_attention(q, cache, shared, softmax_scale=scale, scales=scales), q, cache,
+                  scales, scale)
