@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
   const int2 own_pieces = __ldcg(p.first_piece + b);  // pieces before the sequence, per unit
   const bool first_thread = tid == 0 && blockIdx.z == 0 && blockIdx.y == 0 && blockIdx.x == 0;
   if (first_thread) p.counter[0] = p.counter[1] = 0;
-  if (d4 == 0 && way == 0 && kvh == 0 && (len < shared || len > p.groups.cap_tokens))
+  if (d4 == 0 && way == 0 && kvh == 0 && ((len > 0 && len < shared) || len > p.groups.cap_tokens))
     raise_error(p.err, FAT_DEVERR_BAD_LENGTH);
 
   // Where the row's prefix partials are: the unit's home, or the slots of its CTAs.
@@ -176,10 +176,11 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
 #pragma unroll
   for (int w = 1; w < kJoinWays; ++w) fold(ml_s[w][at], acc_s[w][at]);
 
-  // A sequence without tokens gives zeros (like the decode kernel); a row whose
-  // scores are all -inf has no softmax and gives NaN.
-  const float inv = len > 0 ? 1.f / l : 0.f;
-  const float4 y = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  // A sequence without tokens gives zeros (like the decode kernel), whatever its queries
+  // hold; a row whose scores are all -inf has no softmax and gives NaN.
+  const float inv = 1.f / l;
+  float4 y = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  if (len <= 0) y = make_float4(0.f, 0.f, 0.f, 0.f);
   const long long out_at = (long long)b * p.o_sb + (long long)h * p.o_sh + d4 * 4;
   if (p.out_dtype == FAT_DTYPE_F32) {
     *reinterpret_cast<float4*>(static_cast<float*>(p.out) + out_at) = y;
@@ -327,6 +328,7 @@ int launch_shared_prefix(const SharedPrefixArgs& a) {
   p.groups = Groups{a.cu_groups, a.prefix_lens, a.num_groups, d.batch, d.page_size, cap, std::min(a.max_group, d.batch)};
   p.page_table = d.page_table;
   p.pt_sb = d.pt_sb;
+  p.seq_lens = d.seq_lens;
   p.max_pages = int(d.max_pages);
   p.num_pages = int(d.num_pages);
   p.page_size = d.page_size;

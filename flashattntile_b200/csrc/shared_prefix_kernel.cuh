@@ -160,6 +160,7 @@ struct Params {
   Groups groups;
   const int* page_table;
   long long pt_sb;
+  const int* seq_lens;
   int max_pages, num_pages, page_size, box_rows;
   int num_kv_heads, group, head_dim;
   const float* k_scale;
@@ -487,6 +488,7 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
       Piece w;
       while (ok && walk.next<L::kRowTiles>(p, BN, member, w)) {
         const int* table = p.page_table + (long long)w.first * p.pt_sb;
+        const int first_len = __ldg(p.seq_lens + w.first);
         auto page_of = [&](int j, int& slot0) -> int {
           slot0 = -1;
           const int tok = j * BN + row0;
@@ -507,6 +509,21 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
         };
         int slot1, slot2;
         int page1 = page_of(w.t0, slot1), page2 = page_of(w.t0 + 1, slot2);
+        if (first_len < w.tokens) {
+          // The first sequence does not hold the prefix (any more: it may have been
+          // released); the table is that of the first one that does.
+          for (int i0 = 0; i0 < walk.size; i0 += 32) {
+            const int b = w.first + i0 + lane;
+            const unsigned holds =
+                __ballot_sync(0xffffffffu, i0 + lane < walk.size && __ldg(p.seq_lens + b) >= w.tokens);
+            if (holds != 0u) {
+              table = p.page_table + (long long)(w.first + i0 + __ffs(holds) - 1) * p.pt_sb;
+              break;
+            }
+          }
+          page1 = page_of(w.t0, slot1);
+          page2 = page_of(w.t0 + 1, slot2);
+        }
         page1 = checked(page1, slot1);
         float ks1, vs1;
         scales_of(page1, ks1, vs1);

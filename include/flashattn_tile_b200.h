@@ -432,9 +432,10 @@ int fat_compact_pages(const fat_page_pool* pool, int32_t* table_out, int64_t tab
  *
  * Group g is sequences cu_groups[g] .. cu_groups[g + 1] - 1 (cu_groups int32
  * [num_groups + 1] from 0; sequences past the last group share nothing).  The page
- * tables of a group agree in the first prefix_lens[g] / page_size entries, and none
- * of its sequences is shorter than that many pages (FAT_DEVERR_BAD_LENGTH; the
- * output of a shorter one is then not meaningful).  A prefix that ends inside a page
+ * tables of a group agree in the first prefix_lens[g] / page_size entries; a sequence
+ * of length 0 takes no part (its table is not read, its output is zeros).  Another that
+ * is shorter than that many pages is named (FAT_DEVERR_BAD_LENGTH), and its own output,
+ * not that of the others, is then not meaningful.  A prefix that ends inside a page
  * is used up to the page's start.  No group has more than max_group sequences; one
  * that does is decoded as if it shared nothing (FAT_DEVERR_BAD_GROUP).  Where edges
  * fall (FAT_DEVERR_BAD_GROUP too) the output of the sequences that two groups claim is

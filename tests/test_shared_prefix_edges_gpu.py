@@ -75,3 +75,46 @@ def test_any_scale_on_a_prefix_that_ends_inside_a_tile(kind, rows, dim):
         for scale in (0.0, -0.0, 0.02, -0.3, 1e-38):
             check(shared_prefix_decode_attention(q, cache, shared, softmax_scale=scale, scales=scales), q, cache,
                   scales, scale)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_sequences_that_ended_leave_the_others_right(kind, dim):
+    """Any of a group's sequences may be released, the first ones too: their tables are not
+    read, their outputs are zeros whatever their queries hold, and nothing is reported."""
+    from flashattntile_b200 import find_shared_prefix, shared_prefix_decode_attention, value_checks
+
+    n = 70
+    q, cache, scales = make(kind, [n, 3], [656, 96], [1 + i % 9 for i in range(n + 3)], 8, 4, dim, 16, seed=dim)
+    shared = find_shared_prefix(cache, [n, 3])
+    # Page 0 is what a released row's table holds; here it would do harm.
+    bad = int((set(range(cache.num_pages)) - set(cache.page_table.unique().tolist())).pop())
+    if scales is None:
+        cache.k_cache[bad], cache.v_cache[bad] = float("nan"), float("nan")
+    for ended in ([0], [0, 1, 2, 33], list(range(64)), list(range(1, n)), [n], [n, n + 1], [0, n, n + 2]):
+        lens, table = cache.seq_lens.clone(), cache.page_table.clone()
+        lens[ended], table[ended] = 0, bad
+        now = type(cache)(cache.k_cache, cache.v_cache, table, lens, 16)
+        qs = q.clone()
+        qs[ended] = float("nan")
+        with value_checks(False):
+            out = shared_prefix_decode_attention(qs, now, shared, scales=scales)
+        assert not out[ended].any()
+        check(out, q, now, scales)
+
+
+def test_a_short_sequence_harms_no_other():
+    from flashattntile_b200 import device_error, find_shared_prefix, shared_prefix_decode_attention, value_checks
+
+    q, cache, _ = make("f16", [5], [320], [1, 2, 3, 4, 5], 8, 2, 64, 16, seed=1)
+    shared = find_shared_prefix(cache, [5])
+    want = shared_prefix_decode_attention(q, cache, shared)
+    for short in (0, 2):
+        lens, table = cache.seq_lens.clone(), cache.page_table.clone()
+        lens[short], table[short, 7:] = 100, 0
+        now = type(cache)(cache.k_cache, cache.v_cache, table, lens, 16)
+        with value_checks(False):
+            out = shared_prefix_decode_attention(q, now, shared)
+            assert device_error() == 4
+        rest = [i for i in range(5) if i != short]
+        assert torch.equal(out[rest], want[rest])
