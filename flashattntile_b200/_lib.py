@@ -144,7 +144,7 @@ class PagePoolCall(ctypes.Structure):
         ("scale_stride_page", _i64), ("page_table", _vp), ("page_table_stride", _i64), ("max_pages", _i64),
         ("seq_lens", _vp), ("owned", _vp), ("refs", _vp), ("scratch", _vp), ("scratch_bytes", _sz),
         ("error_word", _vp), ("stream", _vp), ("batch", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
-        ("page_size", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("skip_released", ctypes.c_int32), ("released", _vp),
     ]
 
 

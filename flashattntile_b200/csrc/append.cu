@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   const int b = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hd = a.head_dim;
+  if (a.released != nullptr && __ldg(a.released + b) != 0) return;
   const int pos = a.seq_lens[b];
   const long long cap = (long long)a.max_pages * a.page_size;
   int page = -1, slot = 0;

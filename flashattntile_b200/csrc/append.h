@@ -24,6 +24,7 @@ struct AppendArgs {
   int kv_dtype{}, new_dtype{};
   const int32_t* refs{};               // optional references per page and owned entries per
   const int32_t* owned{};              // sequence: only pages that a sequence alone holds are written
+  const int32_t* released{};           // optional: sequences that are left out (not 0)
   int32_t* error_word{};
   cudaStream_t stream{};
 };

@@ -368,6 +368,8 @@ fat::PageRows rows_of(const fat_page_pool* c) {
   r.owned = c->owned;
   r.refs = c->refs;
   r.batch = c->batch;
+  r.released = c->released;
+  r.skip_released = c->skip_released != 0;
   return r;
 }
 }  // namespace
@@ -433,6 +435,7 @@ int fat_append_to_pool(const fat_page_pool* pool, const void* new_k, const void*
   a.new_dtype = new_dtype;
   a.refs = pool->refs;
   a.owned = pool->owned;
+  a.released = pool->skip_released ? pool->released : nullptr;
   a.error_word = pool->error_word;
   a.stream = static_cast<cudaStream_t>(pool->stream);
   return fat::launch_append_tokens(a);

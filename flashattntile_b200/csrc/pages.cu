@@ -3,7 +3,9 @@
 //
 // State beside the cache: refs[page], how many table entries hold the page
 // (0: free), and owned[row], how many leading entries of a row hold pages (the
-// later entries are 0: a valid page id that is never read).
+// later entries are 0: a valid page id that is never read).  Optionally released[row],
+// 1 from a row's release until it is forked to or reserved by name: a reserve of all rows
+// may leave such rows out, so that a captured step can run while rows are idle.
 // Every operation is defined by whole numbers alone (the lowest free page id
 // first, rows in the order given), so its result does not depend on the order
 // in which threads run: integer counts commute, and every choice is made from
@@ -140,6 +142,8 @@ struct RowParams {
   int* lens;
   int* owned;
   int* refs;
+  int* released;  // null: not kept
+  bool skip_released;
   int batch;
   long long num_pages;
   int page_size;
@@ -233,21 +237,23 @@ __global__ void __launch_bounds__(kBlock) fork_kernel(const RowParams p, const i
   }
   if (!last_block(ticket)) return;
   // All lengths are read before any is written; a row owns what its length
-  // reaches, or the source's own pages when it holds fewer.
+  // reaches, or the source's own pages when it holds fewer.  Length -1 stands for a source
+  // that is released: so is its copy.
   int* len = stage;
   int* own = stage + n;
   for (int d = threadIdx.x; d < n; d += blockDim.x) {
     const int s = __ldcg(src + d);
     const bool ok = row_ok(p, s);
-    len[d] = ok ? max(p.lens[s], 0) : 0;
+    len[d] = ok ? (p.released != nullptr && p.released[s] != 0 ? -1 : max(p.lens[s], 0)) : 0;
     own[d] = ok ? used_pages(p, s) : 0;
   }
   __syncthreads();
   for (int d = threadIdx.x; d < n; d += blockDim.x) {
     const int s = __ldcg(src + d), row = __ldcg(dst + d);
     if (s < 0 || s >= p.batch || !row_ok(p, row) || s == row) continue;
-    p.lens[row] = len[d];
+    p.lens[row] = max(len[d], 0);
     p.owned[row] = own[d];
+    if (p.released != nullptr) p.released[row] = len[d] < 0;
   }
 }
 
@@ -264,6 +270,7 @@ __global__ void __launch_bounds__(kBlock) release_kernel(const RowParams p, cons
   if (threadIdx.x == 0) {
     own_s = min(atomicExch(p.owned + row, 0), p.max_pages);
     p.lens[row] = 0;
+    if (p.released != nullptr) p.released[row] = 1;
   }
   __syncthreads();
   int* at = p.table + (long long)row * p.pt_sb;
@@ -372,7 +379,7 @@ struct Scratch {
 // none), which `held` table entries hold; fresh: pages missing for `tokens` more tokens.
 struct Need {
   int row = -1, at = 0, tail = -1, held = 0, own = 0, fresh = 0;
-  bool ok = false;
+  bool ok = false, idle = false;  // idle: left out on purpose
 };
 
 __device__ __forceinline__ Need row_need(const RowParams& p, const int* rows, int i, int tokens) {
@@ -380,6 +387,8 @@ __device__ __forceinline__ Need row_need(const RowParams& p, const int* rows, in
   const int row = rows != nullptr ? __ldcg(rows + i) : i;
   if (row < 0 || row >= p.batch) return x;
   x.row = row;
+  x.idle = rows == nullptr && p.skip_released && p.released[row] != 0;
+  if (x.idle) return x;
   const int len = p.lens[row];
   x.own = p.owned[row];
   const long long want = ((long long)len + tokens + p.page_size - 1) / p.page_size;
@@ -423,7 +432,7 @@ __global__ void __launch_bounds__(kBlock) reserve_kernel(const RowParams p, cons
   for (int i = tid; i < n; i += kBlock) {
     const Need x = need_of(i);
     if (x.row < 0) raise_error(p.err, FAT_DEVERR_BAD_ROW);
-    else if (!x.ok) raise_error(p.err, FAT_DEVERR_BAD_LENGTH);
+    else if (!x.ok && !x.idle) raise_error(p.err, FAT_DEVERR_BAD_LENGTH);
     if (x.ok && x.tail >= 0) {
       atomicAdd(w.sharers + x.tail, 1);
       atomicMax(w.latest + x.tail, i + 1);
@@ -502,6 +511,7 @@ __global__ void __launch_bounds__(kBlock) reserve_kernel(const RowParams p, cons
       w.pairs[2 * i] = from;
       w.pairs[2 * i + 1] = to;
       if (got && x.ok && x.fresh > 0) p.owned[x.row] = x.own + x.fresh;
+      if (got && x.ok && rows != nullptr && p.released != nullptr) p.released[x.row] = 0;
     }
     // Missing pages, one thread each: offs finds the row of a page.
     offs[tid] = off + (mv ? 1 : 0) - base;
@@ -701,6 +711,8 @@ pg::RowParams row_params(const PageStore& s, const PageRows& r, int32_t* err) {
   p.lens = r.seq_lens;
   p.owned = r.owned;
   p.refs = r.refs;
+  p.released = r.released;
+  p.skip_released = r.skip_released && r.released != nullptr;
   p.batch = r.batch;
   p.num_pages = s.num_pages;
   p.page_size = s.page_size;

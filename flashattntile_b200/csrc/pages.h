@@ -28,6 +28,8 @@ struct PageRows {
   int32_t* owned{};
   int32_t* refs{};
   int batch{};
+  int32_t* released{};  // optional: rows released and not taken up again
+  bool skip_released{}; // a reserve of all rows leaves those out
 };
 
 size_t page_scratch_bytes(int64_t num_pages, int batch);

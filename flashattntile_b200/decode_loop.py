@@ -21,9 +21,12 @@ once for all rows of a group (samples of one prompt, beams):
 
 The captured step is then: make room for a token (a shared tail page is copied),
 append, shared-prefix decode.  Rows may be released and forked, and the pool
-compacted in place, between replays; where that moves group edges or shortens a
-prefix, write the new values into ``shared.cu_groups`` and ``shared.prefix_lens``
-(a prefix shorter than what is shared is always right).  No group may grow past the
+compacted in place, between replays.  A released row is idle: it takes no page and no
+token, and its output is zeros, until it is forked to or reserved by name
+(``pool.reserve(n, rows=...)``).  Where a row takes up other tokens than its group's
+(a new prompt, a fork from another group), write the new edges and prefixes into
+``shared.cu_groups`` and ``shared.prefix_lens`` (a prefix shorter than what is shared is
+always right).  No group may grow past the
 ``max_group`` that ``shared`` had when the loop was made: a larger one is decoded as if
 it shared nothing, and named in the error word.
 
@@ -100,8 +103,8 @@ class DecodeLoop:
     def _append(self):
         c = self.cache
         if self.pool is not None:
-            self.pool.reserve(1)
-            self.pool.append(self.new_k, self.new_v)
+            self.pool.reserve(1, skip_released=True)
+            self.pool.append(self.new_k, self.new_v, skip_released=True)
             return
         launch_append(c.k_cache, c.v_cache, c.page_table, c.seq_lens, self.new_k, self.new_v, c.page_size,
                       k_scale=self.k_scale, v_scale=self.v_scale)

@@ -13,8 +13,10 @@ of one prompt, beams, conversations behind one system prompt:
     pool.compact()                                    # live pages move to the lowest ids
 
 State beside the cache, all on the device: ``refs`` (table entries that hold
-each page; 0: free) and ``owned`` (leading entries of each row that hold pages;
-later entries are 0).  Every operation runs on the current stream without host
+each page; 0: free), ``owned`` (leading entries of each row that hold pages; later
+ones are never read, and 0 where a row has given pages back) and ``released`` (1 for a
+row from its release until it is forked to or reserved by name: a step over all rows
+can leave it out).  Every operation runs on the current stream without host
 synchronisation (with value checks on, the checks read the arguments and the
 outcome back), so a whole serving step can be captured in a CUDA graph.  Results
 are whole numbers that follow from the arguments alone: the lowest free page
@@ -73,6 +75,7 @@ class PagePool:
         self.scales = scales
         self.refs = refs
         self.owned = owned
+        self.released = torch.zeros(cache.batch_size, dtype=torch.int32, device=dev)
         self.live: torch.Tensor | None = None
         lib = _lib.load()
         self._scratch = torch.zeros(lib.fat_page_scratch_size(cache.num_pages, cache.batch_size), dtype=torch.uint8,
@@ -81,6 +84,7 @@ class PagePool:
         c = self._call
         c.page_table, c.page_table_stride, c.max_pages = table.data_ptr(), table.stride(0), table.shape[1]
         c.seq_lens, c.owned, c.refs = lens.data_ptr(), owned.data_ptr(), refs.data_ptr()
+        c.released = self.released.data_ptr()
         c.scratch, c.scratch_bytes, c.batch = self._scratch.data_ptr(), self._scratch.numel(), cache.batch_size
 
     @classmethod
@@ -138,9 +142,12 @@ class PagePool:
         launch("fat_fork_sequences", self._call, dev, src.data_ptr(), dst.data_ptr(), src.numel())
         self._check_outcome("fork")
 
-    def reserve(self, tokens: int = 1, rows: torch.Tensor | None = None) -> None:
+    def reserve(self, tokens: int = 1, rows: torch.Tensor | None = None, skip_released: bool = False) -> None:
         """Make room for ``tokens`` more tokens in each row of ``rows`` (all rows by
-        default): shared, partly filled tail pages are copied, missing pages taken."""
+        default): shared, partly filled tail pages are copied, missing pages taken.
+
+        ``skip_released``, for all rows: those that were released and neither forked to
+        nor reserved by name since take nothing."""
         if not isinstance(tokens, int) or tokens < 0:
             raise ValueError(f"reserve: tokens must be a non-negative integer, got {tokens}")
         dev = self.cache.k_cache.device
@@ -149,20 +156,22 @@ class PagePool:
             rows = check_rows("reserve", rows, dev, "rows")
             n = rows.numel()
             self._check_row_values("reserve", ("rows", rows), distinct="rows")
+        self._call.skip_released = bool(skip_released)
         launch("fat_reserve_tokens", self._call, dev, _lib.ptr(rows), n, tokens)
         self._check_outcome("reserve")
 
     def release(self, rows: torch.Tensor) -> None:
-        """Give the pages of ``rows`` back and empty the rows."""
+        """Give the pages of ``rows`` back and empty the rows (marked in ``released``)."""
         dev = self.cache.k_cache.device
         rows = check_rows("release", rows, dev, "rows")
         self._check_row_values("release", ("rows", rows), distinct="rows")
         launch("fat_release_sequences", self._call, dev, rows.data_ptr(), rows.numel())
         self._check_outcome("release")
 
-    def append(self, new_k: torch.Tensor, new_v: torch.Tensor) -> None:
+    def append(self, new_k: torch.Tensor, new_v: torch.Tensor, skip_released: bool = False) -> None:
         """Append one token per row (``paging.append_tokens``; quantised on write for an
-        8-bit cache), to pages that a row holds alone: ``reserve`` comes first."""
+        8-bit cache), to pages that a row holds alone: ``reserve`` comes first.
+        ``skip_released`` leaves out the rows that ``reserve`` does."""
         c = self.cache
         shape = (c.batch_size, c.num_kv_heads, c.head_dim)
         quant = c.k_cache.dtype in _QUANT
@@ -174,6 +183,7 @@ class PagePool:
             _assert(t.device == c.k_cache.device, f"{name} must be on the cache device")
         if new_k.stride() != new_v.stride() or new_k.stride(2) != 1:
             new_k, new_v = new_k.contiguous(), new_v.contiguous()
+        self._call.skip_released = bool(skip_released)
         launch("fat_append_to_pool", self._call, c.k_cache.device, new_k.data_ptr(), new_v.data_ptr(),
                new_k.stride(0), new_k.stride(1), _lib.DTYPE_CODE[c.k_cache.dtype], _lib.DTYPE_CODE[new_k.dtype])
         self._check_outcome("append")

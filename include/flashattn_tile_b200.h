@@ -368,6 +368,10 @@ int fat_cache_value_stats(const int32_t* seq_lens, const int32_t* page_table, in
  *
  * Strides of the K/V storage are in bytes; row_bytes = head_dim * element size.
  * k_scale/v_scale: optional fp32 [num_pages, num_kv_heads], moved with the pages.
+ * released (optional, int32 [batch], zero at first): 1 for a row from its release until it
+ * is a destination of a fork (which copies the source's mark) or reserved by name.  With
+ * skip_released, fat_reserve_tokens without a row list and fat_append_to_pool leave such
+ * rows as they are: a captured step may run while rows are idle.
  * scratch: fat_page_scratch_size bytes, zero-filled once; every call leaves its
  * counters zero again.  Calls that share a pool are ordered by the caller.
  */
@@ -388,6 +392,8 @@ typedef struct fat_page_pool {
   int32_t* error_word;
   void* stream;
   int32_t batch, num_kv_heads, page_size;
+  int32_t skip_released;
+  int32_t* released;
 } fat_page_pool;
 
 size_t fat_page_scratch_size(int64_t num_pages, int batch);
