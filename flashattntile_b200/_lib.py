@@ -12,9 +12,11 @@ library's ``fat_last_error()``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
+import weakref
 from pathlib import Path
 
 import torch
@@ -95,6 +97,7 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _vp, _vp],
     ),
+    "fat_stream_capture_id": (ctypes.c_uint64, [_vp]),
     "fat_page_scratch_size": (_sz, [_i64, _i32]),
     "fat_copy_pages": (_i32, [_vp, _vp, _vp, _i32]),
     "fat_fork_sequences": (_i32, [_vp, _vp, _vp, _i32]),
@@ -211,31 +214,80 @@ def stream_handle(device: torch.device) -> int:
 
 
 # ---------------------------------------------------------------------------
-# Scratch buffers: one zero-filled buffer per (device, stream), grown on demand.
-# The decode kernel leaves its tickets zeroed on success, so calls ordered on
+# Scratch buffers: one zero-filled workspace and one scratch per (device, stream), grown on
+# demand.  The decode kernel leaves its tickets zeroed on success, so calls ordered on
 # one stream can share the buffer; a call that reported a device error resets it.
+#
+# A CUDA graph goes on using what its calls were given, and nothing tells the library for
+# how long.  So a buffer that is replaced is kept (sizes at least double: all kept ones
+# together are smaller than the one in use), and one that is made during a capture belongs
+# to that capture alone (its zeros are a node of the graph; the graph's own memory pool
+# holds it).  Graphs captured on one stream share its buffers unless they bring their own
+# (own_buffers): replay those one after another.
 # ---------------------------------------------------------------------------
 _WS: dict[tuple[int, int], torch.Tensor] = {}
 _ERR: dict[tuple[int, int], torch.Tensor] = {}
 _SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
 _STATS: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor, torch.cuda.Event]] = {}
+_KEPT: list[torch.Tensor] = []
+_CAPTURED: dict[tuple, tuple[int, torch.Tensor]] = {}
+_LEAST_BYTES = 1 << 16
+
+
+class Buffers:
+    """A workspace and a scratch of their holder's own (a captured loop), for calls on stream ``key``."""
+
+    def __init__(self, key: tuple[int, int]):
+        self.key = key
+        self.workspace: dict[tuple[int, int], torch.Tensor] = {}
+        self.scratch: dict[tuple[int, int], torch.Tensor] = {}
+        _OWNED.add(self)
+
+
+_OWNED: "weakref.WeakSet[Buffers]" = weakref.WeakSet()
+_THREAD = threading.local()
+
+
+@contextlib.contextmanager
+def own_buffers(buffers: Buffers):
+    """Calls of this thread take their workspace and scratch from ``buffers``."""
+    before = getattr(_THREAD, "buffers", None)
+    _THREAD.buffers = buffers
+    try:
+        yield
+    finally:
+        _THREAD.buffers = before
+
+
+def _buffer(held: dict, kind: str, key: tuple[int, int], device: torch.device, nbytes: int) -> torch.Tensor:
+    buf = held.get(key)
+    if buf is not None and buf.numel() >= nbytes:
+        return buf
+    make = torch.zeros if kind == "workspace" else torch.empty
+    nbytes = max(nbytes, _LEAST_BYTES)
+    if torch.cuda.is_current_stream_capturing():
+        capture = load().fat_stream_capture_id(key[1])
+        last, mine = _CAPTURED.get((kind, key), (0, None))
+        if last != capture or mine.numel() < nbytes:
+            mine = make(nbytes, dtype=torch.uint8, device=device)
+            _CAPTURED[(kind, key)] = (capture, mine)
+        return mine
+    if buf is not None:
+        _KEPT.append(buf)
+        nbytes = max(nbytes, 2 * buf.numel())
+    held[key] = buf = make(nbytes, dtype=torch.uint8, device=device)
+    return buf
 
 
 def workspace_for(index: int, stream: int, device: torch.device, nbytes: int) -> torch.Tensor:
-    buf = _WS.get((index, stream))
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-        _WS[(index, stream)] = buf
-    return buf
+    own = getattr(_THREAD, "buffers", None)
+    return _buffer(_WS if own is None else own.workspace, "workspace", (index, stream), device, nbytes)
 
 
 def scratch_for(index: int, stream: int, device: torch.device, nbytes: int) -> torch.Tensor:
     """This stream's scratch without set contents, grown on demand."""
-    buf = _SCRATCH.get((index, stream))
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-        _SCRATCH[(index, stream)] = buf
-    return buf
+    own = getattr(_THREAD, "buffers", None)
+    return _buffer(_SCRATCH if own is None else own.scratch, "scratch", (index, stream), device, nbytes)
 
 
 def error_word_for(index: int, stream: int, device: torch.device) -> torch.Tensor:
@@ -265,6 +317,9 @@ def reset_workspace(device: torch.device) -> None:
     key = _key(device)
     if key in _WS:
         _WS[key].zero_()
+    for own in list(_OWNED):
+        if key in own.workspace:
+            own.workspace[key].zero_()
     if key in _ERR:
         _ERR[key].zero_()
 

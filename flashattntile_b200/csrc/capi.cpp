@@ -21,6 +21,13 @@ const char* fat_last_error(void) { return fat::last_error(); }
 
 uint64_t fat_set_wait_limit_ns(uint64_t limit_ns) { return fat::set_wait_limit_ns(limit_ns); }
 
+uint64_t fat_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id);
+  return e == cudaSuccess && status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 void fat_expire_next_waits(int launches) { fat::request_expiry(launches); }
 
 int fat_set_prefill_p_split(int mode) {

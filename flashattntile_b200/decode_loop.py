@@ -33,7 +33,7 @@ it shared nothing, and named in the error word.
 Nothing on the host depends on the sequence lengths, so every replay sees the
 lengths the previous one left on the device.  A sequence that reaches the end
 of its page table is skipped by the append kernel and reported in the device
-error word (``flashattntile_b200.device_error()``).
+error word of the loop (``loop.device_error()``).
 """
 
 from __future__ import annotations
@@ -87,17 +87,21 @@ class DecodeLoop:
         self.out = torch.empty((b, num_heads, d), dtype=self.q_dtype, device=dev)
         self.stream = torch.cuda.Stream(device=dev)
         self.graph = torch.cuda.CUDAGraph()
+        # Workspace and scratch of the loop's own: streams come from a small pool, so another
+        # loop may be captured on the same one and replayed beside this one.
+        self._buffers = _lib.Buffers(_lib._key(dev)[:1] + (self.stream.cuda_stream,))
         # Library, scratch and error word exist before capture (no allocation,
         # no host synchronisation while capturing); the decode kernel is run
         # once eagerly (it does not change the cache).
         _lib.load()
         self.stream.wait_stream(torch.cuda.current_stream(dev))
-        with _config.value_checks(False), torch.cuda.stream(self.stream):
-            self._decode()
-        self.stream.synchronize()
-        with _config.value_checks(False), torch.cuda.graph(self.graph, stream=self.stream):
-            self._append()
-            self._decode()
+        with _config.value_checks(False), _lib.own_buffers(self._buffers):
+            with torch.cuda.stream(self.stream):
+                self._decode()
+            self.stream.synchronize()
+            with torch.cuda.graph(self.graph, stream=self.stream):
+                self._append()
+                self._decode()
         torch.cuda.current_stream(dev).wait_stream(self.stream)
 
     def _append(self):
@@ -126,6 +130,14 @@ class DecodeLoop:
         self.new_v.copy_(new_v, non_blocking=True)
         self.graph.replay()
         return self.out
+
+    def device_error(self) -> int:
+        """Read and clear what the loop's steps recorded (synchronises): the bits of
+        ``flashattntile_b200.device_error``, in the error word of the stream that the step
+        was captured on."""
+        torch.cuda.synchronize(self.stream.device)
+        with torch.cuda.stream(self.stream):
+            return _lib.read_device_error(self.stream.device)
 
     def replay(self) -> torch.Tensor:
         """Replay with whatever the static buffers ``q``/``new_k``/``new_v`` hold."""

@@ -82,6 +82,11 @@ const char* fat_last_error(void);
  * in-kernel waits. */
 uint64_t fat_set_wait_limit_ns(uint64_t limit_ns);
 
+/* Which capture `stream` is in (a number of its own for each), 0 when it is in none: what a
+ * call of a captured graph is given (workspace, scratch) is that graph's to use for as long
+ * as it is replayed, so a caller keeps it apart from what it hands to other calls. */
+uint64_t fat_stream_capture_id(void* stream);
+
 /* Failure-path testing: each of the next `launches` decode or prefill kernel
  * launches (from any thread) first waits on a barrier phase that nothing
  * completes, so that this wait runs out after the wait limit and the launch

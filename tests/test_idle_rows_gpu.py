@@ -86,9 +86,7 @@ def test_a_loop_goes_on_beside_released_rows(kind, sharing):
     lens[0] = 21
     assert not pool.released.any()
     steps(3)
-    with torch.cuda.stream(loop.stream):
-        assert fat.device_error() == 0
-    assert fat.device_error() == 0
+    assert loop.device_error() == 0 and fat.device_error() == 0
 
 
 def test_marks():
