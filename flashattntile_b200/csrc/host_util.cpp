@@ -132,9 +132,14 @@ bool encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const v
     estride[i] = 1;
     if (i + 1 < rank) gstride[i] = strides_bytes[i];
   }
-  CUresult r = fn(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim, gstride, bdim, estride,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto encode = [&] {
+    return fn(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim, gstride, bdim, estride,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  // A driver call, unlike the runtime's, does not give a thread the device's context: this
+  // may be the thread's first CUDA call.
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaSetDevice(current_device()) == cudaSuccess) r = encode();
   if (r != CUDA_SUCCESS) {
     *why = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(static_cast<int>(r));
     return false;
