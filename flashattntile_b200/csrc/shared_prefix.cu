@@ -2,6 +2,7 @@
 // shared prefix, and the launches (the kernel over the cache is in
 // shared_prefix_kernel.cuh).
 #include <algorithm>
+#include <mutex>
 
 #include "shared_prefix_kernel.cuh"
 
@@ -374,6 +375,10 @@ int launch_shared_prefix(const SharedPrefixArgs& a) {
   o.err = d.error_word;
   o.wait_ns = p.wait_ns;
   p.expire = o.expire = take_expire_request() ? 1 : 0;
+  // The join reads what the kernel before it on the stream left in the scratch: calls of two
+  // threads on one stream go out one after the other.
+  static std::mutex order;
+  const std::lock_guard<std::mutex> lock(order);
   switch (d.kv_dtype) {
     case FAT_DTYPE_F16:
       rc = spx::launch_f16(a, plan, p, o);

@@ -10,6 +10,7 @@ stream's error word (``flashattntile_b200.device_error``).
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -62,7 +63,10 @@ def pool_call(k_cache, v_cache, page_size, k_scale=None, v_scale=None) -> _lib.P
         num_kv_heads=k_cache.shape[2], page_size=int(page_size))
 
 
-def launch(name: str, call: _lib.PagePoolCall, device: torch.device, *args) -> None:
+_LOCK = threading.Lock()
+
+
+def launch(name: str, call: _lib.PagePoolCall, device: torch.device, *args, skip_released: bool = False) -> None:
     """Call library function ``name`` with the struct, on the stream current now."""
     fn = getattr(_lib.load(), name)
     index = device.index if device.index is not None else torch.cuda.current_device()
@@ -70,13 +74,15 @@ def launch(name: str, call: _lib.PagePoolCall, device: torch.device, *args) -> N
     err = _lib._ERR.get((index, stream))
     if err is None:
         err = _lib.error_word_for(index, stream, device)
-    call.stream = stream
-    call.error_word = err.data_ptr()
-    if index == torch._C._cuda_getDevice():
-        status = fn(ctypes.addressof(call), *args)
-    else:
-        with torch.cuda.device(index):
+    with _LOCK:  # the struct is its pool's: from its words to the library's reading of them
+        call.stream = stream
+        call.error_word = err.data_ptr()
+        call.skip_released = skip_released
+        if index == torch._C._cuda_getDevice():
             status = fn(ctypes.addressof(call), *args)
+        else:
+            with torch.cuda.device(index):
+                status = fn(ctypes.addressof(call), *args)
     if status:
         _lib.check(status, name)
 

@@ -18,6 +18,7 @@ sequence's pages on their own).
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass, field
 
 import torch
@@ -53,9 +54,10 @@ class _Packed:
     """The argument struct of a layout -- shapes, strides, types, devices, page size and
     stream -- that passed every structural check, kept in the ``SharedPrefix`` that a
     decode loop holds.  A call with the same layout skips those checks; its pointers
-    are taken from its own tensors, and nothing else of an earlier call is kept."""
+    are taken from its own tensors, and nothing else of an earlier call is kept.  It is
+    the thread's that made it: pointers are written into it before the library reads them."""
 
-    __slots__ = ("layout", "call", "addr", "buffers", "index", "stream")
+    __slots__ = ("layout", "call", "addr", "buffers", "index", "stream", "thread")
 
     @staticmethod
     def layout_of(q, cache, shared, k_scale, v_scale):
@@ -159,7 +161,7 @@ def shared_prefix_decode_attention(q: torch.Tensor, cache: PagedKVCache, shared:
         index = torch._C._cuda_getDevice()
         stream = torch._C._cuda_getCurrentRawStream(index)
         key = (index, stream)
-        if index == packed.index and stream == packed.stream and q.data_ptr() % 16 == 0 \
+        if packed.thread == threading.get_ident() and index == packed.index and stream == packed.stream and q.data_ptr() % 16 == 0 \
                 and packed.layout == _Packed.layout_of(q, cache, shared, k_scale, v_scale) \
                 and _lib._WS.get(key) is packed.buffers[0] and _lib._SCRATCH.get(key) is packed.buffers[1] \
                 and _lib._ERR.get(key) is packed.buffers[2]:
@@ -251,7 +253,7 @@ def shared_prefix_decode_attention(q: torch.Tensor, cache: PagedKVCache, shared:
         packed = _Packed()
         packed.layout = _Packed.layout_of(q, cache, shared, k_scale, v_scale)
         packed.call, packed.addr = call, ctypes.addressof(call)
-        packed.index, packed.stream = idx, stream
+        packed.index, packed.stream, packed.thread = idx, stream, threading.get_ident()
         packed.buffers = (ws, scratch, _lib._ERR[(idx, stream)])
         shared._packed = packed
     return out

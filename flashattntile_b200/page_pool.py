@@ -156,8 +156,7 @@ class PagePool:
             rows = check_rows("reserve", rows, dev, "rows")
             n = rows.numel()
             self._check_row_values("reserve", ("rows", rows), distinct="rows")
-        self._call.skip_released = bool(skip_released)
-        launch("fat_reserve_tokens", self._call, dev, _lib.ptr(rows), n, tokens)
+        launch("fat_reserve_tokens", self._call, dev, _lib.ptr(rows), n, tokens, skip_released=bool(skip_released))
         self._check_outcome("reserve")
 
     def release(self, rows: torch.Tensor) -> None:
@@ -183,9 +182,9 @@ class PagePool:
             _assert(t.device == c.k_cache.device, f"{name} must be on the cache device")
         if new_k.stride() != new_v.stride() or new_k.stride(2) != 1:
             new_k, new_v = new_k.contiguous(), new_v.contiguous()
-        self._call.skip_released = bool(skip_released)
         launch("fat_append_to_pool", self._call, c.k_cache.device, new_k.data_ptr(), new_v.data_ptr(),
-               new_k.stride(0), new_k.stride(1), _lib.DTYPE_CODE[c.k_cache.dtype], _lib.DTYPE_CODE[new_k.dtype])
+               new_k.stride(0), new_k.stride(1), _lib.DTYPE_CODE[c.k_cache.dtype], _lib.DTYPE_CODE[new_k.dtype],
+               skip_released=bool(skip_released))
         self._check_outcome("append")
 
     def compact(self, in_place: bool = True) -> "PagePool":
