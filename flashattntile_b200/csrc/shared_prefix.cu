@@ -292,6 +292,8 @@ int check_shared_prefix(const SharedPrefixArgs& a) {
   if (d.num_heads / d.num_kv_heads > spx::BM)
     return unsupported("shared_prefix_decode: at most " + std::to_string(spx::BM) + " query heads per KV head, got " +
                        std::to_string(d.num_heads / d.num_kv_heads));
+  if (d.num_kv_heads > 65535)  // a dimension of the join's grid
+    return unsupported("shared_prefix_decode: at most 65535 KV heads, got " + std::to_string(d.num_kv_heads));
   const int ob = d.out_dtype == FAT_DTYPE_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(d.out) & 15u) || (d.o_sb * ob) % 16 || (d.o_sh * ob) % 16)
     return unsupported("shared_prefix_decode: out must be 16-byte aligned with 16-byte-multiple strides");
@@ -432,7 +434,12 @@ int launch_shared_prefix(const SharedPrefixArgs& a) {
   // With four ways a block has 8 rows of 32 columns: one per SM from this many values on.
   const bool many = (long long)d.batch * d.num_heads * d.head_dim >= (long long)sm_count(device) * spx::kJoinRows * 32;
   const cudaError_t e = many ? join(spx::join_kernel<4>, 4) : join(spx::join_kernel<16>, 16);
-  if (e != cudaSuccess) return cuda_failure("shared prefix join launch", e);
+  if (e != cudaSuccess) {
+    // Without its join the call leaves pieces counted, and the next call on the workspace
+    // would take them as its own.
+    cudaMemsetAsync(o.counter, 0, 2 * sizeof(int), d.stream);
+    return cuda_failure("shared prefix join launch", e);
+  }
   return FAT_OK;
 }
 
