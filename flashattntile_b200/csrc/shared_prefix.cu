@@ -93,9 +93,8 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
     raise_error(p.err, FAT_DEVERR_BAD_LENGTH);
 
   // Where the row's prefix partials are: the unit's home, or the slots of its CTAs.
-  // With at least a tile per gang these are gangs ca .. cb, of which only the first may
-  // have begun before the unit (its partial is in the CTA's second slot); with fewer,
-  // each tile is a piece.
+  // A gang has at least one tile, so these are gangs ca .. cb, of which only the first may
+  // have begun before the unit (its partial is in the CTA's second slot).
   const long long total = all * p.num_kv_heads;
   const long long u = before * p.num_kv_heads + (long long)kvh * n;
   const bool narrow = (total + 1) * (gangs + 1) < (1ll << 32);
@@ -104,13 +103,13 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
                   : int(((x + 1) * gangs - 1) / total);
   };
   const int ca = n > 0 ? owner(u) : 0, cb = n > 0 ? owner(u + n - 1) : 0;
-  const bool home = ca == cb, dense = total >= gangs;
+  const bool home = ca == cb;
   const long long start =
       n == 0 ? 0 : cut(ca, total, gangs);
   const bool began = n > 0 && start < u;
   const int member = r / p.cta_rows, r_cta = r - member * p.cta_rows;
   const int half = p.parts - 1;  // parts is 1 or 2
-  const int n_prefix = n > 0 ? (home ? 1 : (dense ? cb - ca + 1 : n)) << half : 0;
+  const int n_prefix = n > 0 ? (cb - ca + 1) << half : 0;
   const int first_own = own_pieces.x + (kvh * p.head_groups + hq / own::kRows) * own_pieces.y;
   const int pieces = n_prefix + own_pieces.y;
 
@@ -150,8 +149,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams 
           at_o = p.home_o + ((at * cols + d4) * p.home_rows + R) * 4;
         } else {
           const int j = i >> half, part = i & half;
-          const int c = dense ? ca + j : owner(u + j);
-          const long long at = ((long long)c * p.per_gang + member) * 2 + (began && j == 0 ? 1 : 0);
+          const long long at = ((long long)(ca + j) * p.per_gang + member) * 2 + (began && j == 0 ? 1 : 0);
           const int sr = part * BM + r_cta / p.tile_rows * BM + r_cta % p.tile_rows;
           at_ml = p.slot_ml + (at * 256 + sr) * 2;
           at_o = p.slot_o + ((at * cols + d4) * 256 + sr) * 4;

@@ -57,6 +57,7 @@
 #include "shared_prefix.h"
 #include "shared_prefix_own.cuh"
 #include "tcgen05.cuh"
+#include "widen.cuh"
 
 namespace fat {
 namespace spx {
@@ -297,20 +298,10 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 // Eight 8-bit codes -> eight fp16 values (exact).
 template <KvType kKv>
 __device__ __forceinline__ uint4 widen8(uint2 raw) {
+  using W = Widen<__half, kKv == kKvI8 ? FAT_DTYPE_I8 : FAT_DTYPE_E4M3>;
   uint4 o;
-  if constexpr (kKv == kKvI8) {
-    // u = x + 128: 0x6400 | u is the fp16 number 1024 + u.
-    const uint32_t a = raw.x ^ 0x80808080u, b = raw.y ^ 0x80808080u, magic = 0x64806480u;
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(o.x) : "r"(__byte_perm(a, 0x64646464u, 0x4140)), "r"(magic));
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(o.y) : "r"(__byte_perm(a, 0x64646464u, 0x4342)), "r"(magic));
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(o.z) : "r"(__byte_perm(b, 0x64646464u, 0x4140)), "r"(magic));
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(o.w) : "r"(__byte_perm(b, 0x64646464u, 0x4342)), "r"(magic));
-  } else {
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(o.x) : "h"(uint16_t(raw.x & 0xffffu)));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(o.y) : "h"(uint16_t(raw.x >> 16)));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(o.z) : "h"(uint16_t(raw.y & 0xffffu)));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(o.w) : "h"(uint16_t(raw.y >> 16)));
-  }
+  W::run(raw.x, o.x, o.y);
+  W::run(raw.y, o.z, o.w);
   return o;
 }
 
