@@ -136,11 +136,13 @@ struct Layout {
                 "register split exceeds the launch");
   // What a tile costs a CTA, in units of 32 KB of own tokens.  Swept over sixteen shapes:
   // half or twice them costs up to 50%; over 28 more (head_dim 64 and 128), up to 1.35
-  // times them measures within 3%.  8-bit pairs sit beside a step: 512 rows, 16k shared and
-  // up to 512 own tokens take 106 us, 115 with 3.0, where prefix CTAs come to the own tokens
-  // when a few are left.
+  // times them measures within 3%.  What matters is on which side of a step the whole
+  // units (choose_gangs) fall, and that enough CTAs begin with the own tokens, since a
+  // prefix CTA comes to them late: 512 rows, 16k shared and up to 512 own tokens, int8, take
+  // 105 us, 115 at 3.0; 24 sequences, 16 heads of 64, 16k shared and up to 64 own, fp16,
+  // 24 us, 28 at 1.95.
   static constexpr float kTileCost =
-      (kMode == kRowPair ? (k8 ? 2.6f : 3.8f) : (k8 ? 1.4f : 1.95f)) * (D == 64 ? 0.75f : 1.f);
+      (kMode == kRowPair ? (k8 ? 2.6f : 3.3f) : (k8 ? 1.4f : 1.7f)) * (D == 64 ? 0.75f : 1.f);
   static constexpr int kBars = 4 + 2 * kStagesK + 2 * kStagesV + 6 * kStreams + 3 + 2 * kStagesRaw +
                                (k8 ? kScaleSlots : 0);
   // Per 8 tokens: K scale, log2 of the V scale's size in units, its reciprocal; then the
@@ -1229,7 +1231,8 @@ __global__ void __launch_bounds__(Layout<Types<TQ, KVT, HD>::D, kMode, Types<TQ,
     tiles = 0;
   }
   const int units = p.num_kv_heads * d.head_groups;
-  const float work_p = float(tiles) * p.per_gang * L::kTileCost;
+  constexpr float kCost = L::kTileCost * (std::is_same<typename Y::T, __nv_bfloat16>::value ? 1.15f : 1.f);
+  const float work_p = float(tiles) * p.per_gang * kCost;
   const float work_o = float(tokens) * units * (2.f * LO::kRowBytes / 32768.f);
   const int gangs = choose_gangs(tiles, groups == 1 ? p.num_kv_heads : 0, int(gridDim.x), p.per_gang, work_p, work_o);
   const int piece = own::piece_tokens(tokens, units, d.workers, LO::kTokens);
