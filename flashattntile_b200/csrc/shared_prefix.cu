@@ -46,9 +46,8 @@ constexpr int kJoinThreads = 256;
 // pass before it waits for the kernel before it.
 // kJoinWays threads fold the partials of a row and 4 columns, then together.  Sixteen
 // where four would leave SMs without a block (61 sequences, 8 heads of 64: the whole
-// decode 22.6 us, 24.2 with four; 24 sequences, 16 heads of 64, 16k shared: 29, 35); four
-// elsewhere (64 sequences, 32 heads of 128: 59 us, 82 with sixteen; 8 sequences, 64
-// heads of 128: 113, 116).
+// decode 20.1 us, 21.7 with four); four elsewhere (64 sequences, 32 heads of 128: 56 us, 78
+// with sixteen; 8 sequences, 64 heads of 128: 118, 119).
 template <int kJoinWays>
 __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const JoinParams p) {
   constexpr int kJoinCols = kJoinThreads / kJoinRows / kJoinWays;  // groups of 4 columns of a block

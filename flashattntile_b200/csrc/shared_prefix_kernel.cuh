@@ -33,14 +33,16 @@
 // Every wait is bounded; on a timeout the CTA records FAT_DEVERR_TIMEOUT, drains
 // its copies and MMAs, frees tensor memory and exits.
 //
-// What bounds it, and what it measured (warm, the join included; copies run at 6.5 TB/s):
-//   8 sequences of 133k tokens, 131k shared, 64/8 heads of 128, fp16: 568 MB in 115 us,
-//     4.9 TB/s.  The prefix phase runs at memory speed; 5 us of start, 9 us of join.
-//   64 sequences of 8k + up to 1k tokens, 32/8 heads, bf16: 196 MB in 59 us.  The own
+// What bounds it, and what it measured (one call after another, the join included; copies
+// run at 6.5 TB/s):
+//   8 sequences of 133k tokens, 131k shared, 64/8 heads of 128, fp16: 568 MB in 134 to
+//     140 us, 4.1 TB/s (116 us in short runs of a graph).  5 us of start, 9 us of join; the
+//     second part of P costs 4 to 17 us of it, the more the longer such calls run.
+//   64 sequences of 8k + up to 1k tokens, 32/8 heads, bf16: 196 MB in 60 us.  The own
 //     tokens are two thirds of the bytes: latency of single warps.
-//   128 sequences of 16k + up to 512, 32/8 heads, int8: 101 MB in 101 us: a 16k prefix
-//     against 512 rows is compute, and the softmax of 8-bit tiles (scales per 8 tokens)
-//     takes 1.4 us per unit of both streams, where a 16-bit one takes 0.85.
+//   128 sequences of 16k + up to 512, 32/8 heads, int8: 101 MB in 109 us: a 16k prefix
+//     against 512 rows is compute, in long dependent chains: 40% of the issue slots and 26%
+//     of the tensor pipe are used.
 // MMA issue: one elected thread; a branch on the lane number instead made each MMA cost
 // about 80 cycles of issue, and a unit of both streams 1.6 us instead of 1.05.
 #pragma once
@@ -77,8 +79,9 @@ constexpr long long kMaxTiles = (1ll << 31) - 1;  // tiles on the line (2^38 tok
 
 // Streams: two row tiles, one row tile with half of each tile's tokens each, or one
 // stream.  The rule is the group's rows: up to 128 a second row tile would be empty (an
-// e4m3 case of 32 rows: 59 us, 77 as a pair), past it one row tile per CTA would read and
-// widen every prefix byte once more (512 rows, int8, head_dim 64: 57 us, 62 so).
+// e4m3 case of 32 rows: 59 us, 78 as a pair), past it one row tile per CTA would read and
+// widen every prefix byte once more (512 rows of 16k shared tokens, int8, head_dim 64:
+// 80 us, 91 so).
 enum Mode { kRowPair, kAlternate, kSolo };
 
 enum KvType { kKv16, kKvI8, kKvE4M3 };
@@ -253,7 +256,8 @@ struct Walk {
 // is left out; s0 and s1 sum them in 32 bits.  One part alone costs a result up to as much
 // again as its own rounding to the type, and in 8-bit caches, where P carries the V scale,
 // a group whose scale is far below its neighbours' would vanish from a sum of rounded P.
-// The tensor core has the time.
+// The second product costs nothing where own tokens prevail, 4 to 6% in 8-bit documents and
+// up to 14% where the prefix is most of an fp16 call.
 template <typename T>
 __device__ __forceinline__ uint32_t split_p(float p0, float p1, float& s0, float& s1, uint32_t& rest) {
   constexpr uint32_t kKeep = std::is_same<T, __nv_bfloat16>::value ? 0xffff0000u : 0xffffe000u;
@@ -1144,8 +1148,8 @@ __device__ __forceinline__ void prefix_body(const CUtensorMap& tm_q, const CUten
 // the work a + b.  Whatever the others have left of the own tokens when these are
 // done they share, but nobody can help them: so they are rather many.  A line of one
 // group is cut at its units where that costs little, since every unit a CTA goes on
-// to costs it a query load and a partial more (8 units of 131k tokens: 116 us, 125
-// uncut; where it leaves CTAs idle it costs up to 4%).
+// to costs it a query load and a partial more (8 units of 131k tokens: 117 us, 126
+// uncut; of 32k, 50 and 58; where it leaves CTAs idle it costs up to 2%).
 __device__ __forceinline__ int choose_gangs(long long tiles, int units, int ctas, int per_gang, float a, float b) {
   if (tiles == 0) return 0;
   const int most = int(min(tiles, (long long)max(1, ctas / per_gang)));

@@ -101,10 +101,10 @@ __device__ __forceinline__ int own_tokens(const Groups& g, const int* seq_lens, 
   return max(len - shared, 0);
 }
 
-// Tokens per piece: so many that the warps of the grid get kPiecesPerWarp each (with
-// eight, the partials cost up to 7% more), whole stages, and at least 64: 32 costs a
-// 16k int8 prefix with 512 own tokens 104 us instead of 101, and shorter own parts up to
-// 17%; 128 gains up to 6% there and costs up to 9% where own tokens prevail (balance).
+// Tokens per piece: so many that the warps of the grid get kPiecesPerWarp each (eight
+// measure the same to 1%), whole stages, and at least 64: 32 costs up to 17% (33 sequences
+// of up to 700 own tokens, e4m3: 69.5 us, 59.3); 128 gains up to 3% there and costs up to
+// 5% where own tokens prevail (balance).
 __device__ __forceinline__ int piece_tokens(long long own_total, int units, int workers, int stage) {
   const unsigned long long work = (unsigned long long)own_total * unsigned(units);
   const unsigned parts = unsigned(workers) * kPiecesPerWarp;

@@ -446,7 +446,8 @@ int fat_compact_pages(const fat_page_pool* pool, int32_t* table_out, int64_t tab
  * tables of a group agree in the first prefix_lens[g] / page_size entries; a sequence
  * of length 0 takes no part (its table is not read, its output is zeros).  Another that
  * is shorter than that many pages is named (FAT_DEVERR_BAD_LENGTH), and its own output,
- * not that of the others, is then not meaningful.  A prefix that ends inside a page
+ * not that of the others, is then not meaningful.  Nor is that of a sequence with a page id
+ * outside [0, num_pages), which is not loaded (FAT_DEVERR_BAD_PAGE).  A prefix that ends inside a page
  * is used up to the page's start.  No group has more than max_group sequences; one
  * that does is decoded as if it shared nothing (FAT_DEVERR_BAD_GROUP).  Where edges
  * fall (FAT_DEVERR_BAD_GROUP too) the output of the sequences that two groups claim is
