@@ -265,8 +265,8 @@ def _buffer(held: dict, kind: str, key: tuple[int, int], device: torch.device, n
         return buf
     make = torch.zeros if kind == "workspace" else torch.empty
     nbytes = max(nbytes, _LEAST_BYTES)
-    if torch.cuda.is_current_stream_capturing():
-        capture = load().fat_stream_capture_id(key[1])
+    capture = load().fat_stream_capture_id(key[1]) if key[1] else 0  # the default stream cannot be captured
+    if capture:
         last, mine = _CAPTURED.get((kind, key), (0, None))
         if last != capture or mine.numel() < nbytes:
             mine = make(nbytes, dtype=torch.uint8, device=device)
