@@ -465,7 +465,7 @@ __device__ __forceinline__ void own_body(const CUtensorMap& tm_k, const CUtensor
           const int e = min(253, ((__float_as_int(vm) >> 23) & 0xFF) + 1);
           const float up = __int_as_float(e << 23), a = vunit / up;  // o is 0 before the first unit
           vunit = up;
-          vinv = __int_as_float((254 - e) << 23) * kLift;
+          vinv = __int_as_float((254 - e) << 23);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -473,7 +473,7 @@ __device__ __forceinline__ void own_body(const CUtensorMap& tm_k, const CUtensor
           }
         }
 #pragma unroll
-        for (int r = 0; r < 2 * kSteps; ++r) vf[r] *= vinv;
+        for (int r = 0; r < 2 * kSteps; ++r) vf[r] = vf[r] * vinv * kLift;  // in this order: vinv may be 2^125
       }
       if (__any_sync(0xffffffffu, mx0 > m0 + kRescaleLog2 || mx1 > m1 + kRescaleLog2)) {
 #pragma unroll
