@@ -2,9 +2,9 @@
 // releasing and compacting the pages of a paged KV cache, on the device.
 //
 // State beside the cache: refs[page], how many table entries hold the page
-// (0: free), and owned[row], how many leading entries of a row hold pages (the
-// later entries are 0: a valid page id that is never read).  Optionally released[row],
-// 1 from a row's release until it is forked to or reserved by name: a reserve of all rows
+// (0: free), and owned[row], how many leading entries of a row hold pages (later
+// entries are never read, and become 0, a valid page id, where a row gives pages back).
+// Optionally released[row], 1 from a row's release until it is forked to or reserved by name: a reserve of all rows
 // may leave such rows out, so that a captured step can run while rows are idle.
 // Every operation is defined by whole numbers alone (the lowest free page id
 // first, rows in the order given), so its result does not depend on the order

@@ -364,7 +364,8 @@ int fat_cache_value_stats(const int32_t* seq_lens, const int32_t* page_table, in
  *
  * A pool is a paged K/V cache plus two counts: refs[page], the number of table
  * entries that hold the page (0: free), and owned[row], the number of leading
- * entries of a row that hold pages (later entries are 0).  The operations below
+ * entries of a row that hold pages (later entries are never read; they become 0 where a
+ * row gives pages back).  The operations below
  * keep both exact and run on the device without host synchronisation.  Their
  * results are whole numbers fixed by the arguments alone: the lowest free page
  * ids are taken first, rows are served in the order given.  Row lists hold
